@@ -78,4 +78,26 @@ __device__ __forceinline__ bool mbar_wait_lim(uint64_t* bar, uint32_t parity, ui
 
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
+// The weights p scale_V are held in fp16, against a reference that puts the largest near
+// 2^kPeak when it moves, which it does when one reaches 2^15.  Below 2^-14 fp16 loses bits
+// and below 2^-25 all of them, while the sums l and b keep the whole p: a weight is off by
+// 2^-25 at most, n of them by n 2^-25 against a largest of 2^(kPeak - 1) or more, so the
+// result by n 2^-27 of the largest weight's scale_V (codes within 8 of the middle), 2^-10
+// of a quantisation step behind 131072 tokens.  With the largest at 2^-8, all of fp16 from
+// 1 up idle, an attention sink 12 nats above 131072 others lost a third of the output.
+constexpr float kPeak = 6.f;
+// Scale a value row's weight is taken with: its own, but with room for the sums where it is
+// 0 (equal values, whose codes are 0: any scale stands for them) or next to it.  p stays
+// below 2^95, p min below 2^35.
+constexpr float kScaleMin = 0x1p-80f;
+__device__ __forceinline__ float weight_scale(float s, float mn) {
+  return fmaxf(fmaxf(s, fabsf(mn) * 0x1p-20f), kScaleMin);
+}
+// Largest of weights (two a word, none negative), and whether one reached 2^15 (or is not
+// finite).
+__device__ __forceinline__ uint32_t weight_max(uint32_t m, uint32_t a, uint32_t b) {
+  return __vimax3_u16x2(m, a, b);
+}
+__device__ __forceinline__ bool weight_high(uint32_t m) { return ((m + 0x08000800u) & 0x80008000u) != 0; }
+
 }  // namespace dip

@@ -16,13 +16,12 @@
 // The powers of two go into q (and its row's softmax factor) and into O's rows.
 // q is held in fp16 scaled by a power of two a row (exact for bf16 and fp16
 // elements down to 2^-24 of the row's largest).  The reference M of a row's
-// exponentials is not the largest score but the largest c s + log2 scale_V, plus
-// kRoom: the weights p scale_V that enter the second product in fp16 peak near
-// 2^-kRoom whatever the values' size, and M, l = sum p, b = sum p (min_V + 8 scale_V) and O are
-// rescaled only when a weight reaches 2, which is one bit of the packed weights: a
-// vote a unit, and no reduction over lanes on the usual path.  (fp16 loses bits below
-// 2^-14: 2^-25 a weight at most, against a row sum of 2^-kRoom at least.)  Sums,
-// statistics, pairs and accumulators are fp32.
+// exponentials is not the largest score but the largest c s + log2 scale_V, less
+// kPeak: the weights p scale_V that enter the second product in fp16 peak near
+// 2^kPeak whatever the values' size, and M, l = sum p, b = sum p (min_V + 8 scale_V) and O are
+// rescaled only when a weight reaches 2^15: a maximum of the packed weights and a vote a
+// unit, and no reduction over lanes on the usual path.  (What fp16 loses of small weights:
+// at kPeak.)  Sums, statistics, pairs and accumulators are fp32.
 //
 // Work: the (request, KV head, row block) items are cut into units of 64 cache
 // tokens and laid end to end, each item led by kOvh units that stand for its fixed
@@ -53,9 +52,7 @@ constexpr int kOvh = 2;          // an item's fixed cost in units (queries, firs
 constexpr int kDecMaxReq = 8192;
 constexpr int kDecFineReq = 2048;  // requests with a prefix sum each; above, every fourth has one
 constexpr int kDecInfoReq = 1024;  // requests whose lengths are kept in shared memory
-constexpr float kRoom = 8.f;       // -log2 of the weights' peak after a rescale
 constexpr float kNone = -1e30f;     // reference of a row that has seen no position
-constexpr float kScaleMin = 0x1p-90f;  // smallest scale_V a weight is taken with
 
 template <int D>
 struct DecCfg {
@@ -622,10 +619,7 @@ kv4_decode_kernel(const AttnArgs a, int o_ring, unsigned* __restrict__ counters,
       for (int i = 0; i < TT; ++i) {
         const uint32_t* vp = reinterpret_cast<const uint32_t*>(at_row(i, 4) + tp * (D + 4)) + tau;
 #pragma unroll
-        for (int x = 0; x < 2; ++x) {
-          pair_f32<F16>(vp[8 * x], vs[i][x], vm[i][x]);
-          vm[i][x] = fmaf(8.f, vs[i][x], vm[i][x]);
-        }
+        for (int x = 0; x < 2; ++x) pair_f32<F16>(vp[8 * x], vs[i][x], vm[i][x]);
       }
       if (mask) {
 #pragma unroll
@@ -639,8 +633,8 @@ kv4_decode_kernel(const AttnArgs a, int o_ring, unsigned* __restrict__ counters,
             for (int e = 0; e < 2; ++e)
               if (gone || tok0 + at >= lim[e]) sc[i][e + 2 * x] = -INFINITY;
             // a non-finite value row reaches the rows that see it only (0 * NaN is NaN)
-            if (!(fabsf(vm[i][x]) <= FLT_MAX)) {
-              vm[i][x] = 0.f;
+            if (!(fabsf(vm[i][x]) <= FLT_MAX && vs[i][x] <= FLT_MAX)) {
+              vs[i][x] = vm[i][x] = 0.f;
 #pragma unroll
               for (int e = 0; e < 2; ++e)
                 if (sc[i][e + 2 * x] != -INFINITY) l[e] = __int_as_float(0x7fffffff);
@@ -650,23 +644,27 @@ kv4_decode_kernel(const AttnArgs a, int o_ring, unsigned* __restrict__ counters,
 #pragma unroll
       for (int i = 0; i < TT; ++i)
 #pragma unroll
-        for (int x = 0; x < 2; ++x) vs[i][x] = fmaxf(vs[i][x], kScaleMin);
+        for (int x = 0; x < 2; ++x) {
+          vs[i][x] = weight_scale(vs[i][x], vm[i][x]);
+          vm[i][x] = fmaf(8.f, vs[i][x], vm[i][x]);
+        }
 
       // ---- weights p scale_V
       float p[TT][4];
       uint32_t pw[TT][2];
-      auto weigh = [&]() {  // true: a weight reached 2
-        uint32_t any = 0;
+      auto weigh = [&]() {  // true: a weight reached 2^15
+        uint32_t top = 0;
 #pragma unroll
-        for (int i = 0; i < TT; ++i)
+        for (int i = 0; i < TT; ++i) {
 #pragma unroll
           for (int x = 0; x < 2; ++x) {
 #pragma unroll
             for (int e = 0; e < 2; ++e) p[i][e + 2 * x] = ex2(fmaf(sc[i][e + 2 * x], cf[e], -m[e]));
             pw[i][x] = pack_h2(p[i][2 * x] * vs[i][x], p[i][2 * x + 1] * vs[i][x]);
-            any |= pw[i][x];
           }
-        return (any & 0x40004000u) != 0;
+          top = weight_max(top, pw[i][0], pw[i][1]);
+        }
+        return weight_high(top);
       };
       if (__any_sync(0xffffffffu, weigh())) {
         // too large for the rows' references (always so at first)
@@ -678,7 +676,7 @@ kv4_decode_kernel(const AttnArgs a, int o_ring, unsigned* __restrict__ counters,
           for (int i = 0; i < TT; ++i)
 #pragma unroll
             for (int y = 0; y < 2; ++y)
-              x = fmaxf(x, fmaf(sc[i][e + 2 * y], cf[e], __log2f(vs[i][y]) + kRoom));
+              x = fmaxf(x, fmaf(sc[i][e + 2 * y], cf[e], __log2f(vs[i][y]) - kPeak));
           x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 4));
           x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
           x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16));

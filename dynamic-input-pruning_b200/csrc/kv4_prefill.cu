@@ -14,10 +14,9 @@
 // enter in fp32.  What is rounded: the queries not at all
 // (fp16, scaled by one power of two a tile: exact down to 2^-27 of its largest), the
 // weights p s_V once to fp16, the result once.  A row's reference M (a whole number, so
-// that rescaling is exact) is its largest arg + log2 s_V plus kPfRoom: weights peak
-// near 2^-kPfRoom, and M moves only when one reaches 2, which is one bit of the
-// packed weights (then the tile's earlier weights, O, b and l are rescaled).  fp16
-// loses bits below 2^-14: 2^-25 at most, against a row sum of 2^-kPfRoom at least.
+// that rescaling is exact) is its largest arg + log2 s_V less kPeak: weights peak
+// near 2^kPeak, and M moves only when one reaches 2^15 (then the tile's earlier weights,
+// O, b and l are rescaled).  What fp16 loses of small weights: at kPeak.
 //
 // Warps 0-7: softmax, a warp 32 rows of a block; a thread holds, of each eight columns,
 // two of four rows (the 16x256b shape), so that a pair of columns' pairs (32 bytes) is
@@ -61,8 +60,6 @@ constexpr int kPfPartCost = 8;       // what a part costs beside its steps, in s
 constexpr int kPfWhole = 4;          // rounds of whole tiles from which none is split
 constexpr int kPfCuts = 6;           // ways of cutting that are weighed
 constexpr float kPfNone = -1e30f;    // reference of a row that has seen no position
-constexpr float kPfScaleMin = 0x1p-90f;  // smallest value scale a weight is taken with
-constexpr float kPfRoom = 8.f;       // -log2 of the weights' peak after a rescale
 
 template <int D>
 struct PfCfg {
@@ -552,8 +549,8 @@ kv4_prefill_kernel(const AttnArgs a, int min_rows, int zero_pad, int ctas, PfMet
           };
           uint32_t pk[2][4 * N];
           float lt[4], bt[4];
-          auto weigh = [&]() {  // true: a weight reached 2
-            uint32_t any = 0;
+          auto weigh = [&]() {  // true: a weight reached 2^15
+            uint32_t top = 0;
 #pragma unroll
             for (int e = 0; e < N; ++e) {
               uint32_t w[2][8];
@@ -573,11 +570,11 @@ kv4_prefill_kernel(const AttnArgs a, int min_rows, int zero_pad, int ctas, PfMet
                   bt[r4] = fmaf(y, v.w, first ? x * v.z : fmaf(x, v.z, bt[r4]));
                   const uint32_t p = pf_cvt2<true>(x * v.x, y * v.y);
                   pk[r4 >> 1][4 * e + 2 * g + (r4 & 1)] = p;
-                  any |= p;
+                  if (r4 & 1) top = weight_max(top, p, pk[r4 >> 1][4 * e + 2 * g]);
                 }
               }
             }
-            return (any & 0x40004000u) != 0;
+            return weight_high(top);
           };
           auto rescale = [&]() {
             float nm[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY}, alpha[4];
@@ -589,7 +586,7 @@ kv4_prefill_kernel(const AttnArgs a, int min_rows, int zero_pad, int ctas, PfMet
 #pragma unroll
               for (int g = 0; g < 2; ++g) {
                 const float4 k = par[((c + e) * 2 + g) * 8], v = par[((c + e) * 2 + g) * 8 + 1];
-                const float l0 = __log2f(v.x) + kPfRoom, l1 = __log2f(v.y) + kPfRoom;
+                const float l0 = __log2f(v.x) - kPeak, l1 = __log2f(v.y) - kPeak;
 #pragma unroll
                 for (int r4 = 0; r4 < 4; ++r4) {
                   float x, y;
@@ -788,8 +785,8 @@ kv4_prefill_kernel(const AttnArgs a, int min_rows, int zero_pad, int ctas, PfMet
       const bool bad = seen && !(fabsf(vs) <= FLT_MAX && fabsf(vm) <= FLT_MAX);
       if (!seen) ks = km = 0.f;
       if (!seen || bad) vs = vm = 0.f;
+      vs = weight_scale(vs, vm);
       vm = fmaf(8.f, vs, vm);
-      vs = fmaxf(vs, kPfScaleMin);
       const uint32_t seen_m = __ballot_sync(0xffffffffu, seen), bad_m = __ballot_sync(0xffffffffu, bad);
       if (j >= 2) wait(&kempty[st], ((j >> 1) - 1) & 1);
       if (lane == 0) {
