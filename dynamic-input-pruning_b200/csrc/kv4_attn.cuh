@@ -76,6 +76,14 @@ __device__ __forceinline__ bool mbar_wait_lim(uint64_t* bar, uint32_t parity, ui
   return false;
 }
 
+// For copies and products that are on their way when a wait has run out: they write to, or
+// read, memory that is another block's after this one's exit, so they are waited for with
+// the library's own limit, whatever the caller set.
+__device__ __forceinline__ void mbar_drain(uint64_t* bar, uint32_t parity) {
+  for (uint32_t i = 0; i < kSpinLimit; ++i)
+    if (mbar_try_wait(bar, parity)) return;
+}
+
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
 // The weights p scale_V are held in fp16, against a reference that puts the largest near

@@ -411,8 +411,11 @@ kv4_decode_kernel(const AttnArgs a, int o_ring, unsigned* __restrict__ counters,
   uint32_t badbits = 0;  // four bits a stage: pieces whose page is outside the cache
   const int tp = min(P, kUnit), np = kUnit / tp;  // tokens a piece, pieces a unit
   const int part_bytes = tp * (D + 8);
+  int ahead = 0;       // units asked for and not yet waited for
+  bool dead = false;   // a wait ran out: nothing is loaded any more, the parts are still joined
   auto feed = [&](int st) {
-    if (f_u >= f_end) return;
+    if (f_u >= f_end || dead) return;
+    ++ahead;
     const int t0 = f_u * kUnit;
     const int e = __shfl_sync(0xffffffffu, ent, ((t0 >> pl) - f_page) + (lane & (np - 1)));
     const bool inside = lane < np && t0 + lane * tp < f_kv;
@@ -437,8 +440,6 @@ kv4_decode_kernel(const AttnArgs a, int o_ring, unsigned* __restrict__ counters,
       walk();
     }
   };
-
-  bool dead = false;
 
   constexpr int KW = D / 32;   // packed words a lane and cache row (K), 2 MMA steps each
   constexpr int MT = D / 16;   // m-tiles of O^T
@@ -564,7 +565,18 @@ kv4_decode_kernel(const AttnArgs a, int o_ring, unsigned* __restrict__ counters,
     for (int u = s.u0; u < s.u0 + s.cnt; ++u) {
       __syncwarp();  // the stage before is free
       feed(st == 0 ? S - 1 : st - 1);
-      if (!dead) dead = !mbar_wait_lim(&full[st], par, limit, a.err);
+      if (!dead) {
+        dead = __any_sync(0xffffffffu, !mbar_wait_lim(&full[st], par, limit, a.err));
+        if (dead) {
+#pragma unroll 1
+          for (int i = 0; i < ahead; ++i) {
+            const bool round = st + i >= S;
+            mbar_drain(&full[st + i - (round ? S : 0)], par ^ (round ? 1u : 0u));
+          }
+          __syncwarp();
+        }
+        --ahead;
+      }
       const uint8_t* stage = ring + st * C::stage;
       const int tok0 = u * kUnit;
       const uint32_t bad = (badbits >> (4 * st)) & 15u;

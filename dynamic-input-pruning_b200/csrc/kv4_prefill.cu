@@ -234,7 +234,7 @@ kv4_prefill_kernel(const AttnArgs a, int min_rows, int zero_pad, int ctas, PfMet
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 16);
   uint32_t* masks = reinterpret_cast<uint32_t*>(smem + C::o_mask);
   int* qtop = reinterpret_cast<int*>(bars + 17);   // 16-bit pattern of the tile's largest |q|
-  uint64_t* qbar = bars + 18;
+  uint64_t *qbar = bars + 18, *drain = bars + 19;
   int* plan = reinterpret_cast<int*>(smem + C::o_plan);           // [2][16] scans, tile, part, work
   const int tid = threadIdx.x, lane = tid & 31;
   const int warp = __shfl_sync(0xffffffffu, tid >> 5, 0);  // uniform
@@ -407,6 +407,7 @@ kv4_prefill_kernel(const AttnArgs a, int min_rows, int zero_pad, int ctas, PfMet
       mbar_init(&odone[i], 1);
     }
     mbar_init(qbar, 1);
+    mbar_init(drain, 1);
     *qtop = 0;
     mbar_fence_init();
   }
@@ -420,7 +421,7 @@ kv4_prefill_kernel(const AttnArgs a, int min_rows, int zero_pad, int ctas, PfMet
   __syncthreads();
   pf_fence_after();
   const uint32_t tmem = *tmem_slot;
-  bool dead = false;  // a wait ran out: skip the later ones, free TMEM, return
+  bool dead = false;  // a wait ran out: skip the later ones, drain, free TMEM, return
   auto wait = [&](uint64_t* bar, uint32_t parity) {
     if (!dead) dead = !mbar_wait_lim(bar, parity, limit, a.err);
   };
@@ -858,6 +859,7 @@ kv4_prefill_kernel(const AttnArgs a, int min_rows, int zero_pad, int ctas, PfMet
 #pragma unroll 1
     for (int j = 0; j < nt; ++j) {
       wait(&kfull[j & 1], (j >> 1) & 1);
+      if (__any_sync(0xffffffffu, dead)) break;
 #pragma unroll 1
       for (int t = 0; t < nblk; ++t) {
         if (j > 0) {
@@ -886,7 +888,12 @@ kv4_prefill_kernel(const AttnArgs a, int min_rows, int zero_pad, int ctas, PfMet
   }
   __syncwarp();
   pf_fence_before();
-  __syncthreads();
+  if (__syncthreads_or(dead) && warp == kPfSoft + 4) {  // queries and products still on their way
+    if (pf_elect()) pf_commit(drain);
+    mbar_drain(qbar, 0);
+    mbar_drain(drain, 0);
+    __syncwarp();
+  }
   if (warp == kPfSoft + 4) {
     pf_fence_after();
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;\n" ::"r"(tmem) : "memory");
