@@ -174,7 +174,7 @@ page_release_kernel(const uint8_t* done, int nreq, int page, int32_t* lens, int3
   __shared__ int s_first[kPgThreads], s_held[kPgThreads];
   const int tid = threadIdx.x;
   pdl_wait();
-  int64_t count = *free_count;
+  int64_t count = max(*free_count, 0);  // a negative count is an empty list
   for (int base = 0; base < nreq; base += kPgThreads) {
     const int r = base + tid;
     int held = 0;

@@ -485,7 +485,8 @@ DIP_API int dip_page_extend(const int32_t* lens, const int32_t* new_lens, int64_
                             int32_t* lens_out, int32_t* cu_q, int64_t* slots, int64_t num_tokens,
                             int32_t* free_count_out, int32_t* status, dip_stream_t stream);
 /* Gives the pages of every request with done[r] != 0 back (in request and block
- * order, on top of the free list of capacity free_cap), sets their block table
+ * order, on top of the free list of capacity free_cap; a negative *free_count
+ * counts as 0, pages past the capacity are dropped), sets their block table
  * entries to -1 and their lengths to 0. */
 DIP_API int dip_page_release(const uint8_t* done, int64_t nreq, int64_t page_size, int32_t* lens,
                              int32_t* block_table, int64_t max_blocks, int32_t* free_list,
