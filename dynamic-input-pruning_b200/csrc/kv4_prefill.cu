@@ -428,7 +428,7 @@ kv4_prefill_kernel(const AttnArgs a, int min_rows, int zero_pad, int ctas, PfMet
   constexpr uint32_t kO = 256;  // first column of the O accumulators
 
   // ---------------------------------------------------------------- the tile's queries
-  // one power of two for the tile: largest |q| to [2^13, 2^14)
+  // one power of two for the tile: largest finite |q| to [2^13, 2^14)
   struct RowInfo { float sum; int lim; };  // sum q, positions a row sees
   RowInfo* rowinfo = reinterpret_cast<RowInfo*>(smem + C::o_row);
   constexpr int CH = D / 8, RP = 32 / CH;  // chunks a row, rows a load
@@ -459,9 +459,33 @@ kv4_prefill_kernel(const AttnArgs a, int min_rows, int zero_pad, int ctas, PfMet
     if (lane == 0) atomicMax(qtop, (int)mx);
   }
   __syncthreads();
+  constexpr uint32_t kInf = F16 ? 0x7C00u : 0x7F80u;
+  if (*qtop >= (int)kInf) {  // a row with an infinity or a NaN: the others' scale is not its own
+    __syncthreads();
+    if (tid == 0) *qtop = 0;
+    __syncthreads();
+    if (warp < 8) {
+      uint32_t mx = 0;
+      auto finite = [&](uint32_t w) {
+        const uint32_t lo = w & 0x7FFFu, hi = (w >> 16) & 0x7FFFu;
+        mx = max(mx, max(lo < kInf ? lo : 0u, hi < kInf ? hi : 0u));
+      };
+#pragma unroll 1
+      for (int i = 0; i < CH; ++i) {
+        const uint4 v = q_chunk(warp * 32 + i * RP + lane / CH);
+        finite(v.x);
+        finite(v.y);
+        finite(v.z);
+        finite(v.w);
+      }
+      mx = __reduce_max_sync(0xffffffffu, mx);
+      if (lane == 0) atomicMax(qtop, (int)mx);
+    }
+    __syncthreads();
+  }
   const float qmx = h16_to_f32<F16>((uint32_t)*qtop);
   const int qex = (int)((__float_as_uint(qmx) >> 23) & 255u) - 127;
-  const int qe = qmx > 0.f && qex < 128 ? min(max(13 - qex, -114), 126) : 0;
+  const int qe = qmx > 0.f ? min(max(13 - qex, -114), 126) : 0;
   if (warp < 8) {
     uint8_t* qs = smem + (warp >> 2) * C::block;
     const float sg = pf_pow2(qe);

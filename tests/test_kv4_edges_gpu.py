@@ -29,3 +29,39 @@ def test_page_release_past_the_capacity(dip):
     lens, table = _dev([33]), _dev([[4, 9, 2]])
     dip.page_release(_dev([True], torch.bool), lens, table, free, fc, 16)
     assert room.tolist() == [77, 77, 3, 4] + [77] * 4 and fc.tolist() == [2]
+
+
+def _scaled_keys(seed, L, n, H, hkv, D, P, dtype, size):
+    """Queries of `size` over keys of 1 / size, so that the scores are ordinary ones."""
+    gen = torch.Generator().manual_seed(seed)
+    k = (torch.randn(L, hkv, D, generator=gen) / size).to(dtype)
+    v = torch.randn(L, hkv, D, generator=gen).to(dtype)
+    pages = -(-L // P)
+    cache = torch.zeros(pages, hkv, R.page_bytes(P, D), dtype=torch.uint8)
+    R.put(cache, P, D, dtype, torch.arange(L), k, v)
+    q = (torch.randn(n, H, D, generator=gen) * size).to(dtype)
+    return q, cache.cuda(), torch.arange(pages, dtype=torch.int32, device="cuda").view(1, pages)
+
+
+@pytest.mark.parametrize("bad", [math.nan, math.inf, -math.inf])
+@pytest.mark.parametrize("n", [3, 40, 300])
+@pytest.mark.parametrize("dtype,size", [(BF, 1.0), (BF, 2.0 ** 40), (BF, 2.0 ** -40), (FP, 2.0 ** -12)])
+def test_non_finite_queries_stay_where_they_are(dip, dtype, size, n, bad):
+    """A query with a NaN or an infinity gives NaN; its neighbours' results are their own."""
+    L, H, D, P = 400, 8, 64, 16
+    q, cache, table = _scaled_keys(n, L, n, H, 2, D, P, dtype, size)
+    hit = [(1, 0), (n - 1, 5), (n // 2, 7)]
+    for t, h in hit:
+        q[t, h, 11] = bad
+    q = q.cuda()
+    out, lse = dip.kv4_attention(q, cache, table, _dev([L]), _dev([0, n]), n)
+    picks = sorted({0, 1, n // 2, n - 1})
+    for t, h in hit:
+        assert out[t, h].isnan().all() and lse[t, h].isnan()
+        q[t, h], out[t, h], lse[t, h] = 0, 0, 0
+    ref = T.rows(q, cache, table, [L], [0, n], P, dtype, picks)
+    for t, h in hit:
+        for x in ref.values():
+            x[picks.index(t), h] = 0
+        lse[t, h] = -math.inf
+    T.check(out[picks], lse[picks], ref, dtype)
