@@ -472,6 +472,7 @@ kv4_decode_kernel(const AttnArgs a, int o_ring, unsigned* __restrict__ counters,
     float qsum[2], cf[2];
     int lim[2];
     int minlim = s.kv;
+    bool huge;  // queries so large that 2^24 of their rows' factors is taken by the scores
     uint4 raw[KW];
     const uint16_t* qsrc = q_row(s, lr);
 #pragma unroll
@@ -527,7 +528,8 @@ kv4_decode_kernel(const AttnArgs a, int o_ring, unsigned* __restrict__ counters,
       sum_q += __shfl_xor_sync(0xffffffffu, sum_q, 1);
       sum_q += __shfl_xor_sync(0xffffffffu, sum_q, 2);
       // the rows of this lane's accumulator columns: 2 lc and 2 lc + 1
-      const float c_row = fmaxf(fabsf(a.scale) * kLog2e * pow2i(-qe) * 0x1p24f, FLT_MIN);
+      huge = __any_sync(0xffffffffu, qe < -90);
+      const float c_row = fmaxf(fabsf(a.scale) * kLog2e * pow2i(-qe) * (huge ? 1.f : 0x1p24f), FLT_MIN);
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
         qsum[e] = __shfl_sync(0xffffffffu, sum_q, (2 * lc + e) * 4) * 0x1p-24f;
@@ -580,7 +582,7 @@ kv4_decode_kernel(const AttnArgs a, int o_ring, unsigned* __restrict__ counters,
       const uint8_t* stage = ring + st * C::stage;
       const int tok0 = u * kUnit;
       const uint32_t bad = (badbits >> (4 * st)) & 15u;
-      const bool mask = tok0 + kUnit > minlim || bad;
+      const bool mask = tok0 + kUnit > minlim || bad || huge;
       // tile i's rows: the piece's part, then the rows before it in the piece
       auto at_row = [&](int i, int rb) {
         return stage + ((i * 16) >> tpl) * part_bytes + ((i * 16) & (tp - 1)) * rb;
@@ -634,6 +636,7 @@ kv4_decode_kernel(const AttnArgs a, int o_ring, unsigned* __restrict__ counters,
         for (int x = 0; x < 2; ++x) pair_f32<F16>(vp[8 * x], vs[i][x], vm[i][x]);
       }
       if (mask) {
+        const float up = huge ? 0x1p24f : 1.f;
 #pragma unroll
         for (int i = 0; i < TT; ++i)
 #pragma unroll
@@ -643,7 +646,7 @@ kv4_decode_kernel(const AttnArgs a, int o_ring, unsigned* __restrict__ counters,
             if (gone || tok0 + at >= s.kv) vs[i][x] = vm[i][x] = 0.f;  // rows that nobody wrote
 #pragma unroll
             for (int e = 0; e < 2; ++e)
-              if (gone || tok0 + at >= lim[e]) sc[i][e + 2 * x] = -INFINITY;
+              sc[i][e + 2 * x] = gone || tok0 + at >= lim[e] ? -INFINITY : sc[i][e + 2 * x] * up;
             // a non-finite value row reaches the rows that see it only (0 * NaN is NaN)
             if (!(fabsf(vm[i][x]) <= FLT_MAX && vs[i][x] <= FLT_MAX)) {
               vs[i][x] = vm[i][x] = 0.f;

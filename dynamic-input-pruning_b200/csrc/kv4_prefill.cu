@@ -429,7 +429,7 @@ kv4_prefill_kernel(const AttnArgs a, int min_rows, int zero_pad, int ctas, PfMet
 
   // ---------------------------------------------------------------- the tile's queries
   // one power of two for the tile: largest finite |q| to [2^13, 2^14)
-  struct RowInfo { float sum; int lim; };  // sum q, positions a row sees
+  struct RowInfo { float sum; int lim; };  // sum of the scaled q, positions a row sees
   RowInfo* rowinfo = reinterpret_cast<RowInfo*>(smem + C::o_row);
   constexpr int CH = D / 8, RP = 32 / CH;  // chunks a row, rows a load
   // The rows come by bulk copies, a thread a row, to where keys and values will be: loads in
@@ -499,9 +499,10 @@ kv4_prefill_kernel(const AttnArgs a, int min_rows, int zero_pad, int ctas, PfMet
       for (int j = 0; j < 4; ++j) {
         f[2 * j] = h16_to_f32<F16>(x[j] & 0xFFFFu);
         f[2 * j + 1] = h16_to_f32<F16>(x[j] >> 16);
-        sum_q += f[2 * j] + f[2 * j + 1];
         f[2 * j] *= sg;
-        f[2 * j + 1] *= sg * 0.0625f;  // odd channels: the codes' 16
+        f[2 * j + 1] *= sg;
+        sum_q += f[2 * j] + f[2 * j + 1];
+        f[2 * j + 1] *= 0.0625f;  // odd channels: the codes' 16
       }
       *reinterpret_cast<uint4*>(qs + pf_off<D>(y & 127, lane % CH)) =
           make_uint4(pf_cvt2<true>(f[0], f[4]), pf_cvt2<true>(f[1], f[5]), pf_cvt2<true>(f[2], f[6]),
@@ -799,7 +800,8 @@ kv4_prefill_kernel(const AttnArgs a, int min_rows, int zero_pad, int ctas, PfMet
     load_v();
     entry = page_of(1);
     const int trow = w * 32 + lane;
-    const float fac_m = a.scale * kLog2e, fac_s = fac_m * pf_pow2(-qe) * 0x1p24f;
+    // (the power of two first: with the rest it may be out of range where the pair brings it back)
+    const float fac_q = pf_pow2(-qe), fac_m = a.scale * kLog2e, fac_s = fac_m * 0x1p24f;
 #pragma unroll 1
     for (int j = 0; j < nt; ++j) {
       const int st = j & 1;
@@ -820,8 +822,8 @@ kv4_prefill_kernel(const AttnArgs a, int min_rows, int zero_pad, int ctas, PfMet
       }
       {
         float* p = reinterpret_cast<float*>(smem + C::o_par + (j & 3) * (kPfN * 16)) + (trow >> 1) * 8 + (trow & 1);
-        p[0] = ks * fac_s;
-        p[2] = km * fac_m;
+        p[0] = ks * fac_q * fac_s;
+        p[2] = km * fac_q * fac_m;
         p[4] = vs;
         p[6] = vm;
       }

@@ -65,3 +65,18 @@ def test_non_finite_queries_stay_where_they_are(dip, dtype, size, n, bad):
             x[picks.index(t), h] = 0
         lse[t, h] = -math.inf
     T.check(out[picks], lse[picks], ref, dtype)
+
+
+@pytest.mark.parametrize("n", [1, 3, 40, 300])
+@pytest.mark.parametrize("size", [2.0 ** 119, 2.0 ** 123, 2.0 ** -118])
+@pytest.mark.parametrize("scale", [None, -0.25])
+def test_queries_over_the_whole_range_of_bf16(dip, size, n, scale):
+    """Queries near either end of bf16's range, keys such that the scores are ordinary."""
+    L, H, D, P = 400, 8, 64, 16
+    q, cache, table = _scaled_keys(n, L, n, H, 2, D, P, BF, size)
+    q = q.cuda()
+    out, lse = dip.kv4_attention(q, cache, table, _dev([L]), _dev([0, n]), n, scale=scale)
+    picks = sorted({0, n // 2, n - 1})
+    ref = T.rows(q, cache, table, [L], [0, n], P, BF, picks, scale=scale)
+    assert ref["lse"].isfinite().all() and ref["lse"].abs().max() < 100
+    T.check(out[picks], lse[picks], ref, BF)
