@@ -59,6 +59,29 @@ __device__ __forceinline__ float ex2(float x) {
   return y;
 }
 
+// Tokens of no request, before the first one's and after the last one's: [0, first) and
+// [last, num_tokens).
+struct AttnPad {
+  int first, last;
+};
+__device__ __forceinline__ AttnPad attn_pad(const AttnArgs& a) {
+  if (a.nreq == 0) return {0, 0};
+  const int first = min(max(a.cu_q[0], 0), a.num_tokens);
+  return {first, max(min(a.cu_q[a.nreq], a.num_tokens), first)};
+}
+// Their zeros and -inf, by the whole grid.
+template <int D>
+__device__ __forceinline__ void attn_zero_pad(const AttnArgs& a, const AttnPad& pad, int threads) {
+  const int n = pad.first + (a.num_tokens - pad.last);
+  for (int x = blockIdx.x; x < n; x += gridDim.x) {
+    const int64_t t = x < pad.first ? x : pad.last + (x - pad.first);
+    for (int i = threadIdx.x; i < a.heads * D / 8; i += threads)
+      reinterpret_cast<uint4*>(a.out + t * a.heads * D)[i] = make_uint4(0, 0, 0, 0);
+    if (a.lse)
+      for (int i = threadIdx.x; i < a.heads; i += threads) a.lse[t * a.heads + i] = -INFINITY;
+  }
+}
+
 bool kv4_decode_fits(const AttnArgs& a);
 int kv4_decode(const AttnArgs& a, bool f16, void* counters, void* parts, cudaStream_t st);
 size_t kv4_decode_counter_bytes();

@@ -282,7 +282,7 @@ kv4_decode_kernel(const AttnArgs a, int o_ring, unsigned* __restrict__ counters,
   if (tid == 0) *nfin = 0;
   pdl_wait();
   const uint32_t limit = spin_limit(a.err);  // read once, not in every wait
-  const int pad0 = a.nreq ? a.cu_q[a.nreq] : 0;
+  const AttnPad pad = attn_pad(a);
   // ---------------------------------------------------------------- plan
   // exclusive prefix sums of the requests' costs: each thread a run of requests
   const int gs = a.nreq > kDecFineReq ? 2 : 0;
@@ -902,13 +902,7 @@ kv4_decode_kernel(const AttnArgs a, int o_ring, unsigned* __restrict__ counters,
     }
   }
 
-  // tokens of no request: zeros
-  for (int t = min(max(pad0, 0), a.num_tokens) + blockIdx.x; t < a.num_tokens; t += gridDim.x) {
-    for (int i = tid; i < a.heads * D / 8; i += W * 32)
-      reinterpret_cast<uint4*>(a.out + (int64_t)t * a.heads * D)[i] = make_uint4(0, 0, 0, 0);
-    if (a.lse)
-      for (int i = tid; i < a.heads; i += W * 32) a.lse[(int64_t)t * a.heads + i] = -INFINITY;
-  }
+  attn_zero_pad<D>(a, pad, W * 32);
 }
 
 constexpr int kDecMaxCtas = 160;

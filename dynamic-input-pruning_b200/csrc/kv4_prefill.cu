@@ -372,15 +372,7 @@ kv4_prefill_kernel(const AttnArgs a, int min_rows, int zero_pad, int ctas, PfMet
     }
   __syncthreads();
   pdl_launch_dependents();
-  if (zero_pad) {  // tokens of no request
-    const int t0 = a.nreq ? min(max(a.cu_q[a.nreq], 0), a.num_tokens) : 0;
-    for (int t = t0 + blockIdx.x; t < a.num_tokens; t += gridDim.x) {
-      for (int i = tid; i < a.heads * D / 8; i += kPfThreads)
-        reinterpret_cast<uint4*>(a.out + (int64_t)t * a.heads * D)[i] = make_uint4(0, 0, 0, 0);
-      if (a.lse)
-        for (int i = tid; i < a.heads; i += kPfThreads) a.lse[(int64_t)t * a.heads + i] = -INFINITY;
-    }
-  }
+  if (zero_pad) attn_zero_pad<D>(a, attn_pad(a), kPfThreads);
   const int r = plan[32];
   if (r < 0) return;
   const AttnReq rq = attn_req(a, r);

@@ -80,3 +80,20 @@ def test_queries_over_the_whole_range_of_bf16(dip, size, n, scale):
     ref = T.rows(q, cache, table, [L], [0, n], P, BF, picks, scale=scale)
     assert ref["lse"].isfinite().all() and ref["lse"].abs().max() < 100
     T.check(out[picks], lse[picks], ref, BF)
+
+
+@pytest.mark.parametrize("qs", [[1, 1], [3, 20], [90, 200], [1, 100]])
+@pytest.mark.parametrize("first,after", [(1, 0), (7, 3)])
+def test_tokens_of_no_request(dip, qs, first, after):
+    """Tokens before the first request's and after the last one's: zeros and -inf."""
+    lens, P = [300, 250], 16
+    q, cache, table, cu = _setup(3, lens, qs, 8, 2, 64, P, BF)
+    n = cu[-1]
+    wide = torch.randn(first + n + after, 8, 64, generator=torch.Generator().manual_seed(1)).to(BF)
+    wide[first:first + n] = q
+    junk = torch.full_like(wide, 7.0).cuda()      # leaves something in the allocator's blocks
+    del junk
+    out, lse = _run(dip, wide, cache, table, lens, [x + first for x in cu])
+    R.check(out[first:first + n], lse[first:first + n], R.attention(q, cache, table, lens, cu, P, BF), BF)
+    for part in (slice(0, first), slice(first + n, None)):
+        assert not out[part].any() and lse[part].isinf().all()
