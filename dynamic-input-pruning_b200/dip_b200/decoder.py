@@ -54,16 +54,23 @@ class DipDecoder:
         # norm(x + x) with four times the epsilon: powers of two throughout, so x's own norm to the bit
         return torch.ops.dip_b200.residual_rmsnorm(x, x, 4 * RMS_EPS)
 
-    def _mlp(self, L: dict, x: torch.Tensor) -> torch.Tensor:
-        # as the modules: pruned for few tokens, dense for a prompt's many
-        if x.shape[0] <= _TC_MAX_ROWS:
-            return batched_dip_layer(L, x, self.cfg.k, "tc" if x.shape[0] >= 16 else "gather")[0]
-        return dense_mlp(L["gate_qw"], L["gate_sc"], L["up_qw"], L["up_sc"], L["down_t_qw"],
-                         L["down_t_sc"], x)
+    def _mlp(self, L: dict, x: torch.Tensor, dense: bool) -> torch.Tensor:
+        if dense:
+            return dense_mlp(L["gate_qw"], L["gate_sc"], L["up_qw"], L["up_sc"], L["down_t_qw"],
+                             L["down_t_sc"], x)
+        ys = [batched_dip_layer(L, b, self.cfg.k, "tc" if b.shape[0] >= 16 else "gather")[0]
+              for b in x.split(_TC_MAX_ROWS)]
+        return ys[0] if len(ys) == 1 else torch.cat(ys)
 
-    def step(self, x: torch.Tensor, new_lens: torch.Tensor, max_q: int | None = None) -> torch.Tensor:
+    def step(self, x: torch.Tensor, new_lens: torch.Tensor, max_q: int | None = None,
+             dense: bool = False) -> torch.Tensor:
         """x [tokens, hidden] bf16, new_lens int32 [requests] on the GPU (their sum is
-        tokens, or less where x is padded); max_q bounds one request's new tokens."""
+        tokens, or less where x is padded); max_q bounds one request's new tokens.
+
+        The MLP is pruned for every token, each by its own channels, so that what a
+        request gets does not depend on the requests and tokens that share its step.
+        dense: this step's tokens take all channels, as the reference's modules run
+        prompts (dip_stream_predispatch.py:206-215)."""
         T, c = x.shape[0], self.cache
         h, kv, d = self.heads, self.kv_heads, self.head_dim
         c.extend(new_lens, T, max_q)
@@ -72,7 +79,7 @@ class DipDecoder:
             c.append(l, qkv[:, h:h + kv], qkv[:, h + kv:])
             att, _ = c.attend(l, qkv[:, :h])
             x = x + self.out[l](att.view(T, h * d))
-            x = x + self._mlp(self.mlp[l], self._norm(x))
+            x = x + self._mlp(self.mlp[l], self._norm(x), dense)
         return x
 
     def release(self, done: torch.Tensor) -> None:
@@ -89,7 +96,7 @@ def main() -> None:
     gen = torch.Generator(device=dev).manual_seed(3)
     lens = torch.tensor(prompts, dtype=torch.int32, device=dev)
     x = torch.randn(sum(prompts), cfg.hidden, generator=gen, device=dev).to(torch.bfloat16)
-    y = dec.step(x, lens, max(prompts))
+    y = dec.step(x, lens, max(prompts), dense=True)
     last = y[dec.cache.cu_q[1:].long() - 1]        # the prompts' last tokens
     one = torch.ones_like(lens)
     tok = last.clone()

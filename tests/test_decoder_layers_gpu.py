@@ -4,6 +4,7 @@ import gc
 import pytest
 import torch
 
+import kv4_ref as R
 from test_decoder_gpu import BF, _decoder, _lens, _x
 
 pytestmark = pytest.mark.gpu
@@ -51,3 +52,114 @@ def test_first_step_of_a_length_inside_a_capture(dip):
     with torch.cuda.graph(g):
         dec.step(x, new, 21)
     assert torch.equal(dec.step(x, new, 21), y)
+
+
+# ------------------------------------------------------------- the layers' formula
+
+def _weights(qw, sc, exact):
+    """q * s of signed nibbles, the even column low, a scale for 128 columns: as it is (the
+    GEMVs) or rounded to bf16 (the GEMMs, as dequantize gives it)."""
+    b = qw.view(torch.uint8).long()
+    q = torch.stack([b & 15, b >> 4], -1).flatten(1)
+    w = torch.where(q < 8, q, q - 16).double() * sc.double().repeat_interleave(128, 1)
+    return w if exact else _bf(w)
+
+
+def _bf(x):
+    return x.to(BF).double()
+
+
+def _norm64(x, eps=1e-6):
+    return _bf(x * torch.rsqrt(x.square().mean(-1, keepdim=True) + eps))
+
+
+def _held(x):
+    """What the cache holds of [tokens, heads, D]."""
+    c, s, m = R.quantise(x.to(BF))
+    return c * s[..., None] + m[..., None]
+
+
+def _mlp(L, y, k, exact):
+    g = _bf(torch.nn.functional.silu(_bf(y @ _weights(L["gate_qw"], L["gate_sc"], exact).T)))
+    u = _bf(y @ _weights(L["up_qw"], L["up_sc"], exact).T)
+    kept = g.abs().sort(dim=-1, descending=True, stable=True).indices[:, :k]
+    g = torch.zeros_like(g).scatter(-1, kept, g.gather(-1, kept))
+    return _bf(_bf(g * u) @ _weights(L["down_t_qw"], L["down_t_sc"], exact))
+
+
+def _plain(dec, x, keys, lens, k=None):
+    """One step of requests of `lens` new tokens in 64 bits, every product and sum rounded to
+    bf16 where the layers hand it on.  keys[l][r]: the request's keys and values so far.  k:
+    channels the MLP keeps."""
+    c, h, kv, d = dec.cfg, dec.heads, dec.kv_heads, dec.head_dim
+    x, one = x.double(), x.shape[0] == 1
+    for l in range(c.n_layers):
+        qkv = _bf(_norm64(x) @ _weights(dec.qkv[l].qweight, dec.qkv[l].scales, one).T).view(-1, h + 2 * kv, d)
+        att = torch.zeros(x.shape[0], h, d, dtype=torch.float64, device=x.device)
+        at = 0
+        for r, n in enumerate(lens):
+            sl = slice(at, at + n)
+            new = torch.stack([_held(qkv[sl, h:h + kv]), _held(qkv[sl, h + kv:])])
+            keys[l][r] = torch.cat([keys[l][r], new], 1) if keys[l][r] is not None else new
+            kk, vv = (y.repeat_interleave(h // kv, 1) for y in keys[l][r])
+            s = torch.einsum("ihd,jhd->hij", qkv[sl, :h], kk) / d ** 0.5
+            s.masked_fill_(torch.ones(n, kk.shape[0], device=x.device).triu(kk.shape[0] - n + 1).bool(), -torch.inf)
+            att[sl] = torch.einsum("hij,jhd->ihd", s.softmax(-1), vv)
+            at += n
+        x = _bf(x + _bf(_bf(att).flatten(1) @ _weights(dec.out[l].qweight, dec.out[l].scales, one).T))
+        x = _bf(x + torch.cat([_mlp(dec.mlp[l], y, c.k if k is None else k, y.shape[0] < 16)
+                               for y in _norm64(x).split(128)]))
+    return x
+
+
+def _check(got, want, layers):
+    # The layers and the plain form hand on the same bf16 values but for those that an fp32 sum
+    # puts on the other side of a tie: 64 steps of the tensor cores that cut off 2^-23 each,
+    # 2^-17 against 2^-8, one value in 512, by 2^-8.  Of the cached values 2^-9 * 2^-8 / 0.34
+    # then take another code (a step is 0.34 sigma): 0.34 * sqrt(2.3e-5) = 0.16 % rms where
+    # tokens attend to one position, and up to three times that behind the MLP: 1 % on average.
+    # One row is another matter: a single code of its 256 cached values is 0.34 / 16 = 2.1 %,
+    # two 3 %, and twice that behind the MLP: 6 %.  A second layer whose inputs are off by
+    # 0.5 % takes another code in 0.8 * 0.005 / 0.34 of the cases: 3.7 % rms, 8 % with its MLP.
+    err = (got.double() - want).square().mean(-1).sqrt() / want.square().mean(-1).sqrt()
+    assert err.mean() < (0.01, 0.08)[layers - 1], f"{err.mean():.4f}"
+    assert err.max() < (0.06, 0.12)[layers - 1], f"{err.max():.4f}"
+
+
+def _of(n_layers, requests, tokens, **kw):
+    from dip_b200.decoder import DipDecoder
+    from dip_b200.stack import StackConfig
+    cfg = StackConfig(n_layers=n_layers, seed=5, **{"hidden": 1024, "inter": 2048, **kw})
+    return DipDecoder(cfg, heads=8, kv_heads=2, head_dim=128, max_requests=requests, max_tokens=tokens,
+                      num_pages=requests * (tokens // 16), page_size=16)
+
+
+@pytest.mark.parametrize("layers", [1, 2])
+@pytest.mark.parametrize("steps", [[[50]], [[40, 3, 21], [1, 1, 1], [2, 0, 5]], [[1], [1], [1]]])
+def test_step_is_the_layers_formula(dip, steps, layers):
+    dec = _of(layers, len(steps[0]), 256)
+    keys = [[None] * len(steps[0]) for _ in range(layers)]
+    for i, lens in enumerate(steps):
+        x = _x(sum(lens), 100 + i)
+        _check(dec.step(x, _lens(*lens), max(lens)), _plain(dec, x, keys, lens), layers)
+
+
+@pytest.mark.parametrize("tokens", [50, 200])
+def test_dense_step(dip, tokens):
+    """All channels, for the tokens of the step that asks for it."""
+    dec = _of(1, 1, 256)
+    keys = [[None]]
+    x = _x(tokens, 7)
+    _check(dec.step(x, _lens(tokens), tokens, dense=True), _plain(dec, x, keys, [tokens], dec.cfg.inter), 1)
+    x = _x(1, 8)
+    _check(dec.step(x, _lens(1), 1), _plain(dec, x, keys, [1]), 1)
+
+
+@pytest.mark.parametrize("steps", [[[200], [1]], [[100, 90], [150, 1]], [[1] * 140, [1] * 140]])
+def test_a_token_is_served_alike_in_steps_of_any_size(dip, steps):
+    """Prompts and decode batches of more than 128 tokens are pruned as fewer are."""
+    dec = _of(1, len(steps[0]), 256)
+    keys = [[None] * len(steps[0])]
+    for i, lens in enumerate(steps):
+        x = _x(sum(lens), 100 + i)
+        _check(dec.step(x, _lens(*lens), max(lens)), _plain(dec, x, keys, lens), 1)
