@@ -15,11 +15,12 @@ are synthetic (seeded, quantised int4 g128 as make_layer's).
 from __future__ import annotations
 
 import torch
+import torch.nn.functional as F
 
 from .batch import batched_dip_layer
-from .fastpath import _TC_MAX_ROWS, dense_mlp
+from .fastpath import _TC_MAX_ROWS, dense_mlp, tc_down_ok, tc_linear_ok
 from .kv4 import KV4Cache
-from .qlinear import QuantLinear
+from .qlinear import QuantLinear, dequantize
 from .stack import RMS_EPS, StackConfig, make_layer
 
 
@@ -49,17 +50,33 @@ class DipDecoder:
         self.mlp = [make_layer(cfg, l, device) for l in range(cfg.n_layers)]
         self.cache = KV4Cache(cfg.n_layers, num_pages, kv_heads, head_dim, max_requests,
                               max_tokens, page_size, torch.bfloat16, device)
+        self._mlp_ws = torch.zeros(
+            torch.ops.dip_b200.mlp_workspace_bytes(cfg.hidden, cfg.inter, cfg.k), dtype=torch.uint8,
+            device=device)
 
     def _norm(self, x: torch.Tensor) -> torch.Tensor:
         # norm(x + x) with four times the epsilon: powers of two throughout, so x's own norm to the bit
         return torch.ops.dip_b200.residual_rmsnorm(x, x, 4 * RMS_EPS)
 
     def _mlp(self, L: dict, x: torch.Tensor, dense: bool) -> torch.Tensor:
+        args = (L["gate_qw"], L["gate_sc"], L["up_qw"], L["up_sc"], L["down_t_qw"], L["down_t_sc"])
+        hidden, k = self.cfg.hidden, self.cfg.k
         if dense:
-            return dense_mlp(L["gate_qw"], L["gate_sc"], L["up_qw"], L["up_sc"], L["down_t_qw"],
-                             L["down_t_sc"], x)
-        ys = [batched_dip_layer(L, b, self.cfg.k, "tc" if b.shape[0] >= 16 else "gather")[0]
-              for b in x.split(_TC_MAX_ROWS)]
+            y = dense_mlp(*args, x)
+            if y is None:   # shapes that the GEMMs do not take
+                w = [dequantize(args[i], args[i + 1]) for i in (0, 2, 4)]
+                y = (F.silu(F.linear(x, w[0])) * F.linear(x, w[1])) @ w[2]
+            return y
+        tc = tc_linear_ok(hidden, x) and tc_down_ok(self.cfg.inter, hidden, x)
+        gemv = hidden % 1024 == 0 and hidden <= 5120   # what the batched GEMV takes
+        ys = []
+        for b in x.split(_TC_MAX_ROWS):
+            if tc and (b.shape[0] >= 16 or not gemv):
+                ys.append(batched_dip_layer(L, b, k, "tc")[0])
+            elif gemv:
+                ys.append(batched_dip_layer(L, b, k, "gather")[0])
+            else:   # token by token
+                ys += [torch.ops.dip_b200.mlp_decode(*args, t, k, self._mlp_ws)[0][None] for t in b]
         return ys[0] if len(ys) == 1 else torch.cat(ys)
 
     def step(self, x: torch.Tensor, new_lens: torch.Tensor, max_q: int | None = None,

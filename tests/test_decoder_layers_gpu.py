@@ -87,7 +87,12 @@ def _mlp(L, y, k, exact):
     return _bf(_bf(g * u) @ _weights(L["down_t_qw"], L["down_t_sc"], exact))
 
 
-def _plain(dec, x, keys, lens, k=None):
+def _gemv(hidden, rows):
+    """Whether the pruned MLP of so many tokens runs on the GEMVs: few tokens, or no GEMM for the shape."""
+    return hidden % 256 != 0 or (rows < 16 and hidden % 1024 == 0 and hidden <= 5120)
+
+
+def _plain(dec, x, keys, lens, k=None, exact=_gemv):
     """One step of requests of `lens` new tokens in 64 bits, every product and sum rounded to
     bf16 where the layers hand it on.  keys[l][r]: the request's keys and values so far.  k:
     channels the MLP keeps."""
@@ -107,22 +112,24 @@ def _plain(dec, x, keys, lens, k=None):
             att[sl] = torch.einsum("hij,jhd->ihd", s.softmax(-1), vv)
             at += n
         x = _bf(x + _bf(_bf(att).flatten(1) @ _weights(dec.out[l].qweight, dec.out[l].scales, one).T))
-        x = _bf(x + torch.cat([_mlp(dec.mlp[l], y, c.k if k is None else k, y.shape[0] < 16)
+        x = _bf(x + torch.cat([_mlp(dec.mlp[l], y, c.k if k is None else k, exact(c.hidden, y.shape[0]))
                                for y in _norm64(x).split(128)]))
     return x
 
 
 def _check(got, want, layers):
     # The layers and the plain form hand on the same bf16 values but for those that an fp32 sum
-    # puts on the other side of a tie: 64 steps of the tensor cores that cut off 2^-23 each,
-    # 2^-17 against 2^-8, one value in 512, by 2^-8.  Of the cached values 2^-9 * 2^-8 / 0.34
+    # puts on the other side of a tie: 64 steps of the tensor cores (hidden 1024) that cut off
+    # 2^-23 each, 2^-17 against 2^-8, one value in 512, by 2^-8.  Of the cached values 2^-9 * 2^-8 / 0.34
     # then take another code (a step is 0.34 sigma): 0.34 * sqrt(2.3e-5) = 0.16 % rms where
-    # tokens attend to one position, and up to three times that behind the MLP: 1 % on average.
+    # tokens attend to one position, and up to three times that behind the MLP: 1 % on average
+    # over many rows; with the root of hidden, as the number of such values grows with it.
     # One row is another matter: a single code of its 256 cached values is 0.34 / 16 = 2.1 %,
     # two 3 %, and twice that behind the MLP: 6 %.  A second layer whose inputs are off by
     # 0.5 % takes another code in 0.8 * 0.005 / 0.34 of the cases: 3.7 % rms, 8 % with its MLP.
     err = (got.double() - want).square().mean(-1).sqrt() / want.square().mean(-1).sqrt()
-    assert err.mean() < (0.01, 0.08)[layers - 1], f"{err.mean():.4f}"
+    if err.numel() >= 16:
+        assert err.mean() < (0.01, 0.08)[layers - 1] * (got.shape[1] / 1024) ** 0.5, f"{err.mean():.4f}"
     assert err.max() < (0.06, 0.12)[layers - 1], f"{err.max():.4f}"
 
 
@@ -144,13 +151,25 @@ def test_step_is_the_layers_formula(dip, steps, layers):
         _check(dec.step(x, _lens(*lens), max(lens)), _plain(dec, x, keys, lens), layers)
 
 
+@pytest.mark.parametrize("hidden,inter", [(1152, 2048), (2560, 1024), (1280, 1152), (384, 640), (6144, 512)])
+def test_shapes_that_not_every_kernel_takes(dip, hidden, inter):
+    """Hidden sizes that are no multiple of the GEMMs' 256 or of the batched GEMV's 1024."""
+    dec = _of(1, 2, 512, hidden=hidden, inter=inter)
+    keys = [[None] * 2]
+    for i, (lens, dense) in enumerate([([1, 0], 0), ([3, 2], 0), ([40, 90], 0), ([1, 1], 0), ([60, 1], 1)]):
+        x = torch.randn(sum(lens), hidden, generator=torch.Generator().manual_seed(i)).to(BF).cuda()
+        want = _plain(dec, x, keys, lens, inter if dense else None, (lambda h, n: False) if dense else _gemv)
+        _check(dec.step(x, _lens(*lens), max(lens), dense=bool(dense)), want, 1)
+
+
 @pytest.mark.parametrize("tokens", [50, 200])
 def test_dense_step(dip, tokens):
     """All channels, for the tokens of the step that asks for it."""
     dec = _of(1, 1, 256)
     keys = [[None]]
     x = _x(tokens, 7)
-    _check(dec.step(x, _lens(tokens), tokens, dense=True), _plain(dec, x, keys, [tokens], dec.cfg.inter), 1)
+    _check(dec.step(x, _lens(tokens), tokens, dense=True),
+           _plain(dec, x, keys, [tokens], dec.cfg.inter, lambda h, n: False), 1)
     x = _x(1, 8)
     _check(dec.step(x, _lens(1), 1), _plain(dec, x, keys, [1]), 1)
 
