@@ -51,7 +51,7 @@ extern "C" int dip_residual_rmsnorm(const dip_bf16* y, const dip_bf16* r, int64_
 extern "C" int dip_residual_rmsnorm_rows(const dip_bf16* y, const dip_bf16* r, int64_t rows,
                                          int64_t n, float eps, dip_bf16* out,
                                          dip_stream_t stream) {
-  if (n <= 0 || n > (1 << 20) || rows <= 0 || rows > 65535 || !y || !r || !out) return DIP_ERR_ARG;
+  if (n <= 0 || n > (1 << 20) || rows <= 0 || rows > 0x7fffffffLL || !y || !r || !out) return DIP_ERR_ARG;
   return launch_status(launch(residual_rmsnorm_kernel, dim3((unsigned)rows), dim3(1024), 0,
                               (cudaStream_t)stream, y, r, (int)n, eps, out));
 }

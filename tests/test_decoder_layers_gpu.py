@@ -182,3 +182,17 @@ def test_a_token_is_served_alike_in_steps_of_any_size(dip, steps):
     for i, lens in enumerate(steps):
         x = _x(sum(lens), 100 + i)
         _check(dec.step(x, _lens(*lens), max(lens)), _plain(dec, x, keys, lens), 1)
+
+
+def test_step_of_more_tokens_than_65535(dip):
+    """A prompt of 65600 tokens, and the same one in two steps."""
+    n, cut = 65600, 65000
+    x = _x(n, 9)
+    whole = _of(1, 1, n).step(x, _lens(n), n)
+    dec = _of(1, 1, n)
+    dec.step(x[:cut], _lens(cut), cut)
+    tail = dec.step(x[cut:], _lens(n - cut), n - cut)
+    # each of its tokens attends to 65000 others: what _check allows for codes that differ
+    _check(tail, whole[cut:].double(), 1)
+    norm = dec._norm(x)
+    assert torch.equal(norm[cut:], dec._norm(x[cut:]))
