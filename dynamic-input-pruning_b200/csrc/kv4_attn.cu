@@ -50,11 +50,7 @@ extern "C" int dip_kv4_attention(const dip_kv4_attn_t* p, void* workspace, size_
   a.cache = (const uint8_t*)p->cache;
   a.g = {(int)p->kv_heads, (int)p->head_dim, pl, kv4_part_bytes(p->page_size, p->head_dim),
          p->num_pages};
-  a.table = p->block_table;
   a.max_blocks = p->max_blocks;
-  a.kv_lens = p->kv_lens;
-  a.cu_q = p->cu_q;
-  a.nreq = (int)p->nreq;
   a.num_tokens = (int)p->num_tokens;
   a.heads = (int)p->heads;
   a.group = (int)(p->heads / p->kv_heads);
@@ -64,19 +60,34 @@ extern "C" int dip_kv4_attention(const dip_kv4_attn_t* p, void* workspace, size_
   a.lse = p->lse;
   a.err = error_word_ptr();
   if (!a.err) return launch_status(cudaErrorUnknown);
-  a.max_rows = 0x7fffffff;
   const bool f16 = p->dtype == DIP_FP16;
   cudaStream_t st = (cudaStream_t)stream;
   uint8_t* parts = static_cast<uint8_t*>(workspace) + kv4_decode_counter_bytes();
   const int64_t max_q = std::min(p->max_q, p->num_tokens);
   const bool few = max_q * a.group <= kDecodeRows;
-  // mostly long chunks: the prefill kernel alone; a mixed batch: each request by its kernel
-  if (!few && p->num_tokens * 4 >= p->nreq * max_q) return kv4_prefill(a, f16, 0, true, parts, st);
-  if (!few) a.max_rows = kDecodeRows;
-  if (!kv4_decode_fits(a)) {  // more work than it can number: the other kernel takes any
-    a.max_rows = 0x7fffffff;
-    return kv4_prefill(a, f16, 0, true, parts, st);
-  }
-  const int rc = kv4_decode(a, f16, workspace, parts, st);
-  return rc || few ? rc : kv4_prefill(a, f16, kDecodeRows, false, parts, st);
+  // Every CTA of either kernel goes through all the requests' lengths, so the requests are
+  // taken kMaxReq at a time: 65536 single tokens in one launch took 335 ms, 2^20 would take a
+  // minute and a half.
+  int64_t r0 = 0;
+  do {
+    a.kv_lens = p->kv_lens + r0;
+    a.cu_q = p->cu_q + r0;
+    a.table = p->block_table + r0 * p->max_blocks;
+    a.nreq = (int)std::min<int64_t>(p->nreq - r0, kMaxReq);
+    a.pad = (r0 == 0 ? 1 : 0) | (r0 + a.nreq == p->nreq ? 2 : 0);
+    a.max_rows = few ? 0x7fffffff : kDecodeRows;
+    int rc;
+    // mostly long chunks, or more work than the decode kernel can number: the prefill kernel
+    // alone, which takes any; a mixed batch: each request by its kernel
+    if ((!few && p->num_tokens * 4 >= p->nreq * max_q) || !kv4_decode_fits(a)) {
+      a.max_rows = 0x7fffffff;
+      rc = kv4_prefill(a, f16, 0, true, parts, st);
+    } else {
+      rc = kv4_decode(a, f16, workspace, parts, st);
+      if (!rc && !few) rc = kv4_prefill(a, f16, kDecodeRows, false, parts, st);
+    }
+    if (rc) return rc;
+    r0 += a.nreq;
+  } while (r0 < p->nreq);
+  return DIP_OK;
 }

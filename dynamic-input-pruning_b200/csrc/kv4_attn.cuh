@@ -23,8 +23,10 @@ struct AttnArgs {
   float* lse;
   unsigned* err;
   int max_rows;   // decode kernel: requests with more query rows a KV head are left out
+  int pad;        // tokens of no request that are zeroed: 1 those before the requests', 2 those after
 };
 
+constexpr int kMaxReq = 8192;       // requests a launch
 constexpr int kMaxKv = 0x7fff0000;  // token numbers past a context's end stay 32-bit
 
 // Raises a kernel's dynamic shared memory limit, once a device.
@@ -67,7 +69,8 @@ struct AttnPad {
 __device__ __forceinline__ AttnPad attn_pad(const AttnArgs& a) {
   if (a.nreq == 0) return {0, 0};
   const int first = min(max(a.cu_q[0], 0), a.num_tokens);
-  return {first, max(min(a.cu_q[a.nreq], a.num_tokens), first)};
+  const int last = max(min(a.cu_q[a.nreq], a.num_tokens), first);
+  return {a.pad & 1 ? first : 0, a.pad & 2 ? last : a.num_tokens};
 }
 // Their zeros and -inf, by the whole grid.
 template <int D>

@@ -49,7 +49,6 @@ namespace dip {
 
 constexpr int kUnit = 64;        // cache tokens a unit
 constexpr int kOvh = 2;          // an item's fixed cost in units (queries, first reference, result)
-constexpr int kDecMaxReq = 8192;
 constexpr int kDecFineReq = 2048;  // requests with a prefix sum each; above, every fourth has one
 constexpr int kDecInfoReq = 1024;  // requests whose lengths are kept in shared memory
 constexpr float kNone = -1e30f;     // reference of a row that has seen no position
@@ -932,7 +931,7 @@ bool kv4_decode_fits(const AttnArgs& a) {
   const int64_t units = (std::min<int64_t>(a.max_blocks << a.g.p_log2, kMaxKv) + kUnit - 1) / kUnit + kOvh + 1;
   const int64_t blocks = std::min((int64_t)a.num_tokens * a.group / rows + a.nreq,
                                   ((int64_t)a.max_rows + rows - 1) / rows * a.nreq);
-  return a.nreq <= kDecMaxReq && units * a.g.hkv <= (1LL << 30) / std::max<int64_t>(blocks, 1);
+  return units * a.g.hkv <= (1LL << 30) / std::max<int64_t>(blocks, 1);
 }
 
 int kv4_decode(const AttnArgs& a, bool f16, void* counters, void* parts, cudaStream_t st) {

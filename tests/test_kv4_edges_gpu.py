@@ -97,3 +97,29 @@ def test_tokens_of_no_request(dip, qs, first, after):
     R.check(out[first:first + n], lse[first:first + n], R.attention(q, cache, table, lens, cu, P, BF), BF)
     for part in (slice(0, first), slice(first + n, None)):
         assert not out[part].any() and lse[part].isinf().all()
+
+
+@pytest.mark.parametrize("n,chunk", [(8193, 0), (16384, 0), (20000, 0), (16390, 300)])
+def test_more_requests_than_a_launch_takes(dip, n, chunk):
+    """Requests on both sides of every launch's border, chunks among them; tokens of no request
+    at both ends."""
+    gen = torch.Generator().manual_seed(n)
+    P, D, hkv, H, pages, first, after = 16, 64, 1, 2, 40, 3, 2
+    cache = R.random_cache(gen, pages, hkv, P, D, FP).cuda()
+    table = torch.randint(0, pages, (n, 30), generator=gen, dtype=torch.int32).cuda()
+    lens = torch.randint(0, 48, (n,), generator=gen).tolist()
+    qs = [1] * n
+    for r in (5, 8191, 8192, n - 1) if chunk else ():
+        lens[r], qs[r] = 400, chunk
+    cu = [first]
+    for x in qs:
+        cu.append(cu[-1] + x)
+    q = torch.randn(cu[-1] + after, H, D, generator=gen).to(FP).cuda()
+    out, lse = dip.kv4_attention(q, cache, table, _dev(lens), _dev(cu), max(qs))
+    for part in (slice(0, first), slice(cu[-1], None)):
+        assert not out[part].any() and lse[part].isinf().all()
+    for r in sorted({0, 1, 4, 5, 6, 8190, 8191, 8192, n - 2, n - 1} | set(range(100, n, 997))):
+        L, m = lens[r], qs[r]
+        ref = T.rows(q[cu[r]:cu[r + 1]], cache, table[r:r + 1], [L], [0, m], P, FP, [0, m - 1])
+        sel = [cu[r], cu[r] + m - 1]
+        T.check(out[sel], lse[sel], ref, FP)
