@@ -518,9 +518,10 @@ DIP_API int dip_kv4_read(const void* cache, int64_t num_pages, int64_t page_size
  * kv_heads; query head h reads KV head h / (heads / kv_heads).  out
  * [num_tokens][heads][head_dim], lse [num_tokens][heads] fp32 (natural logarithm
  * of the sum of exponentials; may be NULL).  A query that sees no position, or a
- * token of no request, gets out = 0 and lse = -inf.  Positions past max_blocks
- * pages or in a page outside the cache are not seen.  Sums and softmax
- * statistics are fp32.  Queries are multiplied in fp16, scaled by a power of two for a
+ * token of no request, gets out = 0 and lse = -inf.  A kv_lens[r] beyond max_blocks
+ * pages counts as that many tokens (the queries' positions are counted back from it);
+ * positions in a page outside the cache are not seen.  cu_q ascends and stays within
+ * num_tokens.  Sums and softmax statistics are fp32.  Queries are multiplied in fp16, scaled by a power of two for a
  * row (few rows) or for up to 256 rows of a request's KV head (chunks): exact for
  * elements down to 2^-24 and 2^-27 of the largest of these.  max_q is the caller's
  * bound on the query tokens of one request; it only chooses the kernel (too small a
