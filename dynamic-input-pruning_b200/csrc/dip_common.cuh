@@ -237,6 +237,7 @@ namespace dip {
 #endif
 constexpr uint32_t kSpinLimit = DIP_SPIN_LIMIT;
 constexpr unsigned kErrTimeout = 1u;
+constexpr unsigned kErrInput = 2u;  // an input on the device that the kernel refuses
 // `err` points at the library's device control block (error_word_ptr):
 // word 0 holds the error bits, word 1 the poll limit of the bounded waits
 // (0: kSpinLimit; set with dip_set_spin_limit).

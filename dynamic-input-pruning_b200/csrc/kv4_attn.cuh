@@ -46,11 +46,13 @@ inline cudaError_t attn_smem(int bytes) {
 // Request r: first query token, query tokens (clamped to the call's), visible cache length.
 struct AttnReq {
   int tok0, n, kv;
+  bool bad;  // cu_q descends: the sums of n that both kernels count with are not bounded then
 };
 __device__ __forceinline__ AttnReq attn_req(const AttnArgs& a, int r) {
   AttnReq q;
   q.tok0 = max(a.cu_q[r], 0);
   q.n = max(min(a.cu_q[r + 1], a.num_tokens) - q.tok0, 0);
+  q.bad = a.cu_q[r + 1] < a.cu_q[r];
   q.kv = (int)min((int64_t)min(max(a.kv_lens[r], 0), kMaxKv), a.max_blocks << a.g.p_log2);
   return q;
 }

@@ -281,16 +281,18 @@ kv4_decode_kernel(const AttnArgs a, int o_ring, unsigned* __restrict__ counters,
   if (tid == 0) *nfin = 0;
   pdl_wait();
   const uint32_t limit = spin_limit(a.err);  // read once, not in every wait
-  const AttnPad pad = attn_pad(a);
+  AttnPad pad = attn_pad(a);
   // ---------------------------------------------------------------- plan
   // exclusive prefix sums of the requests' costs: each thread a run of requests
   const int gs = a.nreq > kDecFineReq ? 2 : 0;
   const int per = (((a.nreq + C::threads - 1) / C::threads) + (1 << gs) - 1) >> gs << gs;
   int sum = 0, aligned = 0;  // costs in the two ways of laying the items out
+  bool bad_cu = false;
   for (int i = 0; i < per; ++i) {
     const int r = tid * per + i;
     if (r < a.nreq) {
       const AttnReq q = attn_req(a, r);
+      bad_cu |= q.bad;
       if (r < kDecInfoReq) {
         info[3 * r] = q.tok0;
         info[3 * r + 1] = q.n;
@@ -314,7 +316,7 @@ kv4_decode_kernel(const AttnArgs a, int o_ring, unsigned* __restrict__ counters,
     scan[warp] = inc;
     scan[16 + warp] = inc2;
   }
-  __syncthreads();
+  bad_cu = __syncthreads_or(bad_cu);
   int before = inc - sum, before2 = inc2 - aligned, total = 0, total2 = 0;
 #pragma unroll
   for (int w = 0; w < W; ++w) {
@@ -333,6 +335,11 @@ kv4_decode_kernel(const AttnArgs a, int o_ring, unsigned* __restrict__ counters,
   if (sh.few) {
     before = before2;
     total = total2;
+  }
+  if (bad_cu) {  // no work, all tokens zeros
+    total = 0;
+    pad = {0, 0};
+    if (blockIdx.x == 0 && tid == 0) atomicOr(a.err, kErrInput);
   }
   const int share = max((total + workers - 1) / workers, 1);
   for (int i = 0; i < per; ++i) {

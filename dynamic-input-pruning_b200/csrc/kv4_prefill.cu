@@ -321,9 +321,11 @@ kv4_prefill_kernel(const AttnArgs a, int min_rows, int zero_pad, int ctas, PfMet
   }
   auto parts_of = [&](const AttnReq& q) { return SPLIT ? max((steps_of(q.kv) + span - 1) / span, 1) : 1; };
   int sum = 0, split = 0;  // parts of this thread's requests; of split tiles
+  bool bad_cu = false;
   for (int i = 0; i < per; ++i)
     if (tid * per + i < a.nreq) {
       const AttnReq q = attn_req(a, tid * per + i);
+      bad_cu |= q.bad;
       const int np = parts_of(q), n = tiles_of(q) * np;
       sum += n;
       if (np > 1) split += n;
@@ -342,7 +344,8 @@ kv4_prefill_kernel(const AttnArgs a, int min_rows, int zero_pad, int ctas, PfMet
     plan[16 + warp] = inc2;
   }
   if (tid == 0) plan[32] = -1;
-  __syncthreads();
+  bad_cu = __syncthreads_or(bad_cu);  // then no tile, all tokens zeros
+  if (bad_cu && blockIdx.x == 0 && tid == 0) atomicOr(a.err, kErrInput);
   int before = inc - sum, split_before = inc2 - split;
   for (int w = 0; w < warp; ++w) {
     before += plan[w];
@@ -351,9 +354,9 @@ kv4_prefill_kernel(const AttnArgs a, int min_rows, int zero_pad, int ctas, PfMet
   if (SPLIT && blockIdx.x == 0 && tid == 0) {
     int all = 0;
     for (int w = 0; w < NW; ++w) all += plan[16 + w];
-    meta[kPfSlots].r = all * a.g.hkv;
+    meta[kPfSlots].r = bad_cu ? 0 : all * a.g.hkv;
   }
-  if (sum > 0 && want >= before && want < before + sum)
+  if (!bad_cu && sum > 0 && want >= before && want < before + sum)
     for (int i = 0; i < per; ++i) {
       const int r = tid * per + i;
       if (r >= a.nreq) break;
@@ -372,7 +375,7 @@ kv4_prefill_kernel(const AttnArgs a, int min_rows, int zero_pad, int ctas, PfMet
     }
   __syncthreads();
   pdl_launch_dependents();
-  if (zero_pad) attn_zero_pad<D>(a, attn_pad(a), kPfThreads);
+  if (zero_pad) attn_zero_pad<D>(a, bad_cu ? AttnPad{0, 0} : attn_pad(a), kPfThreads);
   const int r = plan[32];
   if (r < 0) return;
   const AttnReq rq = attn_req(a, r);

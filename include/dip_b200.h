@@ -53,7 +53,8 @@ DIP_API const char* dip_last_cuda_error(void);
 DIP_API int dip_set_pdl(int enable);
 /* Reads and clears the device error word of the current device: bit 0 set
  * means a kernel gave up a bounded wait (a pipeline barrier that never
- * completed) and returned early; its outputs are then invalid.  Synchronous
+ * completed) and returned early; its outputs are then invalid; bit 1 that one
+ * refused an input on the device (dip_kv4_attention: cu_q descends).  Synchronous
  * (a device-to-host copy).  0 = no error recorded. */
 DIP_API int dip_take_device_error(unsigned int* out);
 /* Sets the poll limit of every bounded device wait (grid barriers, the fused
@@ -520,8 +521,8 @@ DIP_API int dip_kv4_read(const void* cache, int64_t num_pages, int64_t page_size
  * of the sum of exponentials; may be NULL).  A query that sees no position, or a
  * token of no request, gets out = 0 and lse = -inf.  A kv_lens[r] beyond max_blocks
  * pages counts as that many tokens (the queries' positions are counted back from it);
- * positions in a page outside the cache are not seen.  cu_q ascends and stays within
- * num_tokens.  Sums and softmax statistics are fp32.  Queries are multiplied in fp16, scaled by a power of two for a
+ * positions in a page outside the cache are not seen.  cu_q ascends; where it does not,
+ * no query is served (out = 0, lse = -inf) and bit 1 of the device error word is set.  Sums and softmax statistics are fp32.  Queries are multiplied in fp16, scaled by a power of two for a
  * row (few rows) or for up to 256 rows of a request's KV head (chunks): exact for
  * elements down to 2^-24 and 2^-27 of the largest of these.  max_q is the caller's
  * bound on the query tokens of one request; it only chooses the kernel (too small a

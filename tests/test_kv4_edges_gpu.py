@@ -123,3 +123,27 @@ def test_more_requests_than_a_launch_takes(dip, n, chunk):
         ref = T.rows(q[cu[r]:cu[r + 1]], cache, table[r:r + 1], [L], [0, m], P, FP, [0, m - 1])
         sel = [cu[r], cu[r] + m - 1]
         T.check(out[sel], lse[sel], ref, FP)
+
+
+@pytest.mark.parametrize("cu,max_q", [
+    ([0, 5, 3, 20], 17), ([0, 20, 0, 20], 20), ([0, 200, 100, 200], 200), ([20, 10, 5, 0], 1),
+    ([0, 200] * 40, 200), ([0, 3] * 500, 1), ([0, 200] * 4, 1),
+])
+@pytest.mark.parametrize("D", [64, 128])
+def test_a_descending_cu_q_is_refused(dip, cu, max_q, D):
+    """It is known on the device only: zeros, and the device error word."""
+    n = len(cu) - 1
+    lens = [300] * n
+    q, cache, table, _ = _setup(n, [300], [200], 8, 2, D, 64, BF)
+    ws = dip.kv4_workspace("cuda")
+    args = (q.cuda(), cache.cuda(), table.cuda().repeat(n, 1))
+    take = torch.ops.dip_b200.take_device_error
+    assert take() == 0
+    out, lse = dip.kv4_attention(*args, _dev(lens), _dev(cu), max_q, workspace=ws)
+    assert take() == 2
+    assert not out.any() and lse.isinf().all()
+    good = [0, 200]
+    out, lse = dip.kv4_attention(args[0], args[1], table.cuda(), _dev([300]), _dev(good), 200, workspace=ws)
+    ref = R.attention(q, cache, table, [300], good, 64, BF)
+    R.check(out, lse, ref, BF)
+    assert take() == 0
