@@ -14,9 +14,9 @@ using namespace dip;
 
 // Up to this many query rows a KV head the decode kernel is faster, which reads the cache
 // once for eight; the prefill kernel's cost hardly depends on them.  Decode / prefill, us:
-// 16 contexts of 900 to 9000 tokens, 8 heads of 128: 143 / 174 at 64 rows, 170 / 176 at 80,
-// 198 / 178 at 96, 256 / 180 at 128; 60 of 500: 79 / 118, -, 107 / 120, 131 / 122; one of
-// 60000: -, 121 / 124 at 72, 150 / 124, 195 / 124.
+// 16 contexts of 900 to 9000 tokens, 8 heads of 128: 145 / 191 at 64 rows, 174 / 191 at 80,
+// 203 / 194 at 96, 262 / 196 at 128; 60 of 500: 80 / 118, 94 / 118, 109 / 120, 133 / 122; one
+// of 60000: 123 / 123 at 72, 154 / 122 at 96, 199 / 122 at 128.
 static constexpr int kDecodeRows = 80;
 
 extern "C" size_t dip_kv4_attention_workspace_bytes(void) {

@@ -12,7 +12,7 @@
 // row (two 16-byte words, half a row apart): what is done once a row is shared by them.
 // A warp takes kKvBatch x 32 lanes of one token's key and value rows, all loads first.
 // Measured, 65521 tokens, 8 heads of 128, bf16 (340 MB each way): append 88 us, 3.9 TB/s;
-// read 58 us, 5.9 TB/s or 90 % of a measured 6.5 TB/s copy.  64 tokens: 3 us each, launch.
+// read 58 us, 5.9 TB/s or 90 % of a measured 6.5 TB/s copy.  64 tokens: 2 us each, launch.
 #include <cfloat>
 
 #include "kv4_common.cuh"

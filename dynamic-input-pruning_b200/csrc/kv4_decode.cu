@@ -34,11 +34,11 @@
 // the CTA that completes an item's count of parts joins them in fixed order.
 // Bound by HBM (0.53 bytes a cached element); every warp streams its own units into
 // a ring of shared memory, one bulk copy a page (a page of one head is contiguous).
-// Measured, 64/8 heads of 128, bf16: one context of 131071 tokens 43 us, 3.3 TB/s or 51 %
+// Measured, 64/8 heads of 128, bf16: one context of 131071 tokens 44 us, 3.3 TB/s or 50 %
 // of a measured copy (the stream itself 25 us, 5.7 TB/s; the rest plan, first units and the
-// joins); 64 contexts of 17 to 16384 43 us; one of 700 10 us with the launch.  256 contexts
-// of 1 to 2048, 8 heads of 64, fp16: 29 us, by the items' fixed latency.  16 x 5 tokens of
-// 40/8 heads behind 900 to 9000: 55 us, by unpacking for each of four row blocks.
+// joins); 64 contexts of 17 to 16384 44 us; one of 700 10 us with the launch.  256 contexts
+// of 1 to 2048, 8 heads of 64, fp16: 30 us, by the items' fixed latency.  16 x 5 tokens of
+// 40/8 heads behind 900 to 9000: 56 us, by unpacking for each of four row blocks.
 #include <algorithm>
 #include <cfloat>
 #include <type_traits>

@@ -12,7 +12,7 @@
 // the rounding of a weight weighs no more than its value, the neighbour nibble's times
 // 16; the factor 16 is taken out of the queries and of O's columns), and the pairs
 // enter in fp32.  What is rounded: the queries not at all
-// (fp16, scaled by one power of two a tile: exact down to 2^-27 of its largest), the
+// (fp16, scaled by one power of two a tile: exact down to 2^-27 of its largest finite one), the
 // weights p s_V once to fp16, the result once.  A row's reference M (a whole number, so
 // that rescaling is exact) is its largest arg + log2 s_V less kPeak: weights peak
 // near 2^kPeak, and M moves only when one reaches 2^15 (then the tile's earlier weights,
@@ -24,14 +24,14 @@
 // in registers.  Warp 12: issues the MMAs, in the order P0 V, Q0 K, P1 V, Q1 K of
 // successive tiles, so that one block's softmax runs under the other's products.
 //
-// Few tiles or a long one among them: tiles are cut along the keys into parts, each to a slot
-// of the workspace (M, l, O + b of its rows in fp32), which a second kernel joins in their
-// order.  32 tokens behind 300000, 64/8 heads: 0.47 ms (whole 6.98); 2 x 200 behind 30000,
-// 32/4 heads: 0.47 ms (whole 0.72).  A launch that cuts nothing pays 5 to 20 us for the
-// choice (700 fresh tokens 46 and 41 us, 4000 257 and 239), so those with four rounds of
-// tiles or more go without.
+// In a call with tokens for fewer than four rounds of tiles, few tiles or a long one among
+// them are cut along the keys into parts, each to a slot of the workspace (M, l, O + b of its
+// rows in fp32), which a second kernel joins in their order.  32 tokens behind 300000, 64/8
+// heads: 0.47 ms (whole 7.02); 2 x 200 behind 30000, 32/4 heads: 0.47 ms (whole 0.72).  A
+// launch that cuts nothing pays for the choice (700 fresh tokens 59 and 51 us), so calls with
+// more tokens go without, also where one of their contexts is long.
 //
-// Measured: 4096 tokens behind 4096, 64/8 heads of 128, bf16, 1.12 ms, 0.74 PFLOP/s or
+// Measured: 4096 tokens behind 4096, 64/8 heads of 128, bf16, 1.12 ms, 0.73 PFLOP/s or
 // 44 % of a measured 1.66 PFLOP/s matrix product.  Bound by the softmax warps' latency
 // and issue: 4150 of a tile's 5700 cycles in the softmax, 1300 waiting for the block's
 // own products (1024 at the tensor cores' rate); and by about eight steps a tile for finding
