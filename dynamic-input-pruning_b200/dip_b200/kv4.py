@@ -78,9 +78,9 @@ def kv4_attention(q, cache, block_table, kv_lens, cu_q, max_q: int, scale: float
     """q [tokens, heads, head_dim] over the cache -> (out like q, lse [tokens, heads]).
 
     Request r's queries q[cu_q[r]:cu_q[r+1]] are the last of its kv_lens[r] cached
-    tokens.  scale defaults to 1 / sqrt(head_dim).  max_q bounds the query tokens
-    of one request; it only chooses the kernel.  A query that sees nothing gets
-    zeros and lse -inf.  Without a workspace (kv4_workspace) each call makes one."""
+    tokens; cu_q ascends (else no query is served and take_device_error() gives 2).  scale defaults to 1 / sqrt(head_dim).  max_q bounds the query tokens
+    of one request; it only chooses the kernel.  A query that sees nothing, or of no
+    request, gets zeros and lse -inf.  Without a workspace (kv4_workspace) each call makes one."""
     if scale is None:
         scale = 1.0 / math.sqrt(q.shape[-1])
     return torch.ops.dip_b200.kv4_attention.default(q, cache, block_table, kv_lens, cu_q, max_q,
